@@ -227,8 +227,7 @@ def _prepare_sample(case, seed, gen, dev):
 def run(s):
     kind = s["case"]["kind"]
     if kind == "plan":
-        n, T = s["case"]["adapters"], s["T"]
-        cap = T // TILE + min(s["adapter"].shape[0], n + 1)  # from what the program has in hand
+        n, T, cap = s["case"]["adapters"], s["T"], _item_cap(s["case"])
         if own:
             from flashqwen_amd.lora import lora_plan
 
