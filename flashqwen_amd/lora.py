@@ -131,8 +131,10 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     """out = y + the adapters' products, row by row of the plan, on the current stream: y [rows,
     n_out] bf16 or fp32 (what the projection left), x [rows, n_in] bf16 (row strides allowed), a
     [n, slices * rank_max, n_in] and b [n, n_out, rank_max] bf16, scale [n] fp32, rank [n] int32
-    (default: rank_max for all).  `out` may be y (in place, rows without an adapter untouched);
-    without it a new tensor is returned, whose rows that the plan does not hold are undefined."""
+    (default: rank_max for all).  `out` may be y (in place, rows without an adapter untouched).
+    Rows that the plan does not hold, and rows of adapters that a and b do not have, are left as
+    they were in `out`; without it a new tensor is returned, a copy of y that the products are
+    added to, so these rows are y's there (the copy is a pass of its own over y)."""
     index = x.get_device()
     bf16 = torch.bfloat16
     f32 = y.dtype is torch.float32
@@ -167,7 +169,8 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     if T == 1:  # the row stride of a single row may be anything
         ldx, ldy = K, N
     if out is None:
-        out, ldo = torch.empty(T, N, dtype=y.dtype, device=x.device), N
+        y = out = y.detach().clone(memory_format=torch.contiguous_format)
+        ldy = ldo = N
     elif out is y:
         ldo = ldy
     else:
