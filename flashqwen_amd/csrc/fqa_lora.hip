@@ -525,23 +525,26 @@ struct Out<true> {
   typedef float T;
 };
 
-// The parts of v as bf16: v = hi + mid (to 16 bits and more), + lo (to all of fp32's).  An infinity
-// has no parts but the first.
+// The parts of v as bf16: the sum of two is v to 2^-16 of its value, of three all of it.  Every part has
+// v's sign and is zero only if v is (above 2^-100), so that a product with an infinity is that
+// infinity from each: bits are cut off, not rounded, before the last part, and a value that leaves
+// nothing for the next part shares itself with it.  An infinity or a NaN is each of its parts.
 template <int kParts>
 __device__ __forceinline__ void split_bf16(float v, uint16_t (&part)[kParts]) {
 #pragma unroll
-  for (int p = 0; p < kParts; ++p) {
-    part[p] = f32_to_bf16_bits(v);
-    const float g = bf16_bits_to_f32(part[p]);
-    v = __builtin_fabsf(g) < INFINITY ? v - g : 0.f;
+  for (int p = 0; p < kParts - 1; ++p) {
+    const uint32_t all = __float_as_uint(v), cut = all & 0xffff0000u;
+    const float g = __uint_as_float(cut) * (all == cut ? 0.5f : 1.f);
+    part[p] = (uint16_t)(__float_as_uint(g) >> 16);
+    v = (all & 0x7f800000u) == 0x7f800000u ? v : v - bf16_bits_to_f32(part[p]);
   }
+  part[kParts - 1] = f32_to_bf16_bits(v);
 }
-typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 
 // y = y_in + scale h B^T.  A wave has 64 columns at a time of an item's rows, 16 rows to an MFMA.  One
 // MFMA multiplies 16 ranks: its k 0..15 are h's first bf16 parts, 16..31 its second ones, against
-// B's 16 values twice, so that h keeps 16 bits and more (one bf16 would round it to 8); for an fp32
-// y another one adds the third parts.  Four MFMAs give a lane 16 consecutive columns of one row:
+// B's 16 values twice, so that h keeps 16 bits (one bf16 would round it to 8); for an fp32 y another
+// one adds the halves of the third parts, twice.  Four MFMAs give a lane 16 consecutive columns of one row:
 // row i of B that MFMA m takes is column 16 (i / 4) + 4 m + i % 4 of the 64.
 template <bool kF32>
 struct Expand {
@@ -613,6 +616,7 @@ struct Expand {
       for (int e = 0; e < 4; ++e) {
         uint16_t x[kParts];
         split_bf16(j + e < rk ? v[e] * scale : 0.f, x);
+        if constexpr (kF32) x[2] = f32_to_bf16_bits(0.5f * bf16_bits_to_f32(x[2]));
 #pragma unroll
         for (int k = 0; k < kParts; ++k) part[k][e] = (short)x[k];
       }
@@ -625,11 +629,10 @@ struct Expand {
   __device__ __forceinline__ void multiply(const bf16x8 (&f)[4], int rb, int jb, float4_t (&acc)[4]) const {
     const char* p = lds + (rb * 16 + li) * pitch + (q & 1) * 16 + jb * 32;
     if constexpr (kF32) {
-      u16x8 z = *reinterpret_cast<const u16x8*>(p + 4 * a.R);
-      if (q >> 1) z = 0;
+      const bf16x8 z = *reinterpret_cast<const bf16x8*>(p + 4 * a.R);
 #pragma unroll
       for (int m = 0; m < 4; ++m)
-        acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[m], __builtin_bit_cast(bf16x8, z), acc[m], 0, 0, 0);
+        acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[m], z, acc[m], 0, 0, 0);
     }
     const bf16x8 hf = *reinterpret_cast<const bf16x8*>(p + (q >> 1) * a.R * 2);
 #pragma unroll

@@ -565,7 +565,8 @@ int fqa_lora_plan(const int32_t* adapter, int32_t n_ids, const int32_t* req_map,
  * or fp32.  y may be y_in (with the same stride): rows without an adapter are then left alone,
  * otherwise they are copied.  y must not overlap x, the weights or y_in in any other way.  Rows
  * that the plan does not hold are not written.  All sums are fp32; scale (x A^T) enters the
- * second product as two bf16 (its value to 16 bits and more), three for an fp32 y.  item_bound <=
+ * second product as two bf16 (its value to 2^-16), three for an fp32 y (all of its value); infinities
+ * of x, a, b and y_in give the infinities and NaNs that the formula gives.  item_bound <=
  * FQA_LORA_MAX_ITEMS: items from it on are ignored, and so are those of an adapter that w does not
  * have.  ldx a multiple of 8, ldyi and ldy of 4 elements; x, a, b, y_in, y, items and workspace
  * 16-byte aligned.  `workspace`: fqa_lora_workspace_bytes(w, rows_bound, item_bound) bytes, no
