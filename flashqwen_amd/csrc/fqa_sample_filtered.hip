@@ -30,7 +30,7 @@
 // both on fp64 weights; a dozen more of 0.5 to 2).  256 rows greedy 35, of top_k 20 46, without a
 // filter 54, of every kind 75 (gather 15, pick 22).  64 rows 43 (scan 12, merge 7, gather 7, pick 20).
 // One row: greedy 7, top_k 20 17, top-p 29, launches of 1.5 us and the pick's chain.  Rows that
-// select_row does take 380 to 620.
+// select_row does take 410 to 650.
 #include "fqa_common.h"
 
 #include <cfloat>
@@ -52,7 +52,6 @@ struct FilterArgs {
   const float* min_p;
   const float* u;
   int32_t* out;
-  int unit;  // select_row's masses are in units of 2^-unit
   int rows, parts;  // parts of a row (0: no scan)
   int4* head;           // [rows][parts] {largest key, its lowest index, list length, highest bin}
   unsigned long long* body;  // [rows][parts][kBody]
@@ -180,13 +179,64 @@ __device__ u64 block_sum(u64 n, BlockLds& sh) {
   return z;
 }
 
+// A mass in two words, in units of 2^-38 and 2^-76 of the largest weight: a double's weight down to
+// 2^-76, and the sums of up to 2^24 weights fit each word by itself, so that they are exact in any
+// order.  (One word would leave a vocabulary of 2^24 no more than 2^-39: a tail of weights below half
+// of that, which together may be 3e-5, would count as nothing.)  Counts go in the first word.
+constexpr int kMassBits = 38;
+typedef unsigned __int128 u128;
+struct Mass {
+  u64 hi, lo;
+  __device__ __forceinline__ u128 value() const { return ((u128)hi << kMassBits) + lo; }
+};
+__device__ __forceinline__ Mass mass_from(double w) {  // w in [0, 1]
+  const double s = ldexp(w, kMassBits), whole = floor(s);
+  return {(u64)whole, (u64)ldexp(s - whole, kMassBits)};
+}
+struct MassLds {
+  u64 hi[kFBins], lo[kFBins];
+  u64 wlo[kFWaves];
+  u64 above[2];
+};
+// As crossing, of masses.
+__device__ int crossing_mass(MassLds& m, BlockLds& sh, u128 need, u128& above) {
+  const int t = threadIdx.x, lane = t & (kWave - 1), w = t >> 6;
+  const int b0 = kFBins - 1 - 2 * t;
+  const Mass m0{m.hi[b0], m.lo[b0]}, m1{m.hi[b0 - 1], m.lo[b0 - 1]};
+  const Mass incl{wave_scan64(m0.hi + m1.hi), wave_scan64(m0.lo + m1.lo)};
+  if (lane == kWave - 1) {
+    sh.wsum[w] = incl.hi;
+    m.wlo[w] = incl.lo;
+  }
+  if (t == 0) sh.bin = 0;
+  __syncthreads();
+  Mass ahead{incl.hi - m0.hi - m1.hi, incl.lo - m0.lo - m1.lo};
+  for (int i = 0; i < w; ++i) {
+    ahead.hi += sh.wsum[i];
+    ahead.lo += m.wlo[i];
+  }
+  const u128 before = above + ahead.value(), with0 = before + m0.value(), with1 = with0 + m1.value();
+  if (before < need && with1 >= need) {
+    const bool first = with0 >= need;
+    sh.bin = first ? b0 : b0 - 1;
+    const u128 over = first ? before : with0;
+    m.above[0] = (u64)over;
+    m.above[1] = (u64)(over >> 64);
+  }
+  __syncthreads();
+  above = (u128)m.above[1] << 64 | m.above[0];
+  const int bin = sh.bin;
+  __syncthreads();
+  return bin;
+}
+
 // A row by a whole 1024-thread workgroup, straight from the logits: every selection is a radix
-// select over the keys (11, 11, 10 bits), counts or masses (in units of 2^-unit of the largest
-// weight) in an LDS histogram.  The row is not greedy and has a logit above -inf (mk).  A function
-// of its own, out of the way of the code that nearly every row runs.
+// select over the keys (11, 11, 10 bits), counts or masses in an LDS histogram.  The row is not
+// greedy and has a logit above -inf (mk).  A function of its own, out of the way of the code that
+// nearly every row runs.
 __device__ __noinline__ int select_row(const float* lg, int N, uint32_t mk, double it, int k_top,
-                                       double p, double min_w, double u, int unit) {
-  __shared__ u64 hist[kFBins];
+                                       double p, double min_w, double u) {
+  __shared__ MassLds hist;
   __shared__ BlockLds sh;
   const int t = threadIdx.x, lane = t & (kWave - 1);
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -205,29 +255,40 @@ __device__ __noinline__ int select_row(const float* lg, int N, uint32_t mk, doub
   };
   const double M = (double)logit_of(mk);
   auto weight = [&](uint32_t k) { return k == mk ? 1.0 : exp(((double)logit_of(k) - M) * it); };
-  auto mass = [&](uint32_t k) { return (u64)(ldexp(weight(k), unit) + 0.5); };
+  auto mass = [&](uint32_t k) { return mass_from(weight(k)); };
   // the cut: kept are keys above ck, and of those equal the indexes up to ci
   uint32_t ck = kKeyMasked + 1;
   int ci = N;
   auto kept = [&](uint32_t k, int i) { return k > ck || (k == ck && i <= ci); };
   // the prefix of what is kept whose `value`s sum to `need` or more: a new cut
-  auto select = [&](u64 need, auto&& value) {
+  auto select = [&](u128 need, auto&& value) {
     uint32_t prefix = 0;
-    u64 above = 0;
+    u128 above = 0;
     for (int level = 0; level < 3; ++level) {
       const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11;
-      for (int b = t; b < kFBins; b += kFThreads) hist[b] = 0;
+      for (int b = t; b < kFBins; b += kFThreads) hist.hi[b] = hist.lo[b] = 0;
       __syncthreads();
       for_each([&](uint32_t k, int i) {
-        if (kept(k, i) && (level == 0 || (k >> (shift + bits)) == prefix))
-          atomicAdd(&hist[k >> shift & ((1u << bits) - 1)], value(k));
+        if (kept(k, i) && (level == 0 || (k >> (shift + bits)) == prefix)) {
+          const Mass v = value(k);
+          const uint32_t b = k >> shift & ((1u << bits) - 1);
+          atomicAdd(&hist.hi[b], v.hi);
+          if (v.lo) atomicAdd(&hist.lo[b], v.lo);
+        }
       });
       __syncthreads();
-      prefix = prefix << bits | (uint32_t)crossing(hist, sh, need, above);
+      prefix = prefix << bits | (uint32_t)crossing_mass(hist, sh, need, above);
     }
-    // of the elements with this key, the first q
-    const u64 one = value(prefix);
-    const u64 q = one ? (need - above + one - 1) / one : 1;
+    // of the elements with this key, the first q: as many as reach what is left
+    const Mass one = value(prefix);
+    const u128 each = one.value(), rest = need - above;
+    u64 q = 1;
+    if (each) {  // the quotient in fp64, then made exact
+      const auto f = [](u128 x) { return ldexp((double)(u64)(x >> 64), 64) + (double)(u64)x; };
+      q = (u64)fmin(fmax(f(rest) / f(each), 1.0), (double)N);
+      while (q < (u64)N && each * q < rest) ++q;
+      while (q > 1 && each * (q - 1) >= rest) --q;
+    }
     u64 n = 0;
     for_each([&](uint32_t k, int i) { n += k == prefix && kept(k, i) ? 1 : 0; });
     n = wave_sum64(n);
@@ -255,16 +316,26 @@ __device__ __noinline__ int select_row(const float* lg, int N, uint32_t mk, doub
     ci = sh.pick;
     __syncthreads();
   };
-  auto total = [&](auto&& value) {
+  if (k_top > 0) {
     u64 n = 0;
-    for_each([&](uint32_t k, int i) { n += kept(k, i) ? value(k) : 0; });
-    return block_sum(n, sh);
-  };
-  const auto one = [](uint32_t) { return 1ull; };
-  if (k_top > 0 && total(one) > (u64)k_top) select((u64)k_top, one);
+    for_each([&](uint32_t k, int i) { n += kept(k, i) ? 1 : 0; });
+    if (block_sum(n, sh) > (u64)k_top)
+      select((u128)k_top << kMassBits, [](uint32_t) { return Mass{1, 0}; });
+  }
   if (p < 1.0) {
-    const u64 need = (u64)ceil(p * (double)total(mass));
-    select(need > 0 ? need : 1, mass);
+    Mass all{0, 0};
+    for_each([&](uint32_t k, int i) {
+      if (!kept(k, i)) return;
+      const Mass v = mass(k);
+      all.hi += v.hi;
+      all.lo += v.lo;
+    });
+    all.hi = block_sum(all.hi, sh);
+    all.lo = block_sum(all.lo, sh);
+    // p times it in units of 2^-38 (p <= 1 - 2^-24, so that rounding does not take it past all)
+    const double share = p * ((double)all.hi + ldexp((double)all.lo, -kMassBits)), whole = floor(share);
+    const u128 need = ((u128)(u64)whole << kMassBits) + (u64)ceil(ldexp(share - whole, kMassBits));
+    select(need > 0 ? need : (u128)1, mass);
   }
   // the pick
   auto kept_weight = [&](uint32_t k, int i) {
@@ -1412,7 +1483,7 @@ __global__ void __launch_bounds__(kFThreads) filter_pick_kernel(FilterArgs a) {
   __syncthreads();
   // the token in one lane, -1 in the others
   const int token = select_row(a.logits + (long long)row * a.stride, a.vocab, mk, st.it, st.k, st.p,
-                               st.min_w, st.u, a.unit);
+                               st.min_w, st.u);
   if (token >= 0) a.out[row] = token;
 }
 
@@ -1452,11 +1523,9 @@ extern "C" int fqa_sample_filtered(const float* logits, int32_t n_rows, int32_t 
   if (!logits || !inv_temp || !top_k || !top_p || !min_p || !u || !out ||
       (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))))
     return FQA_EINVAL;
-  int bits = 0;
-  while ((1 << bits) < vocab) ++bits;
   const int parts = scan_parts(vocab);
-  FilterArgs a{logits, vocab, row_stride, inv_temp, top_k, top_p, min_p, u, out,
-               62 - bits < 44 ? 62 - bits : 44, n_rows, parts, (int4*)workspace,
+  FilterArgs a{logits, vocab, row_stride, inv_temp, top_k, top_p, min_p, u, out, n_rows, parts,
+               (int4*)workspace,
                (u64*)((char*)workspace + (int64_t)n_rows * parts * 16),
                (RowBins*)((char*)workspace + (int64_t)n_rows * parts * (16 + 8 * kBody))};
   const hipStream_t st = (hipStream_t)stream;
