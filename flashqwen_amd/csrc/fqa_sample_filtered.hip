@@ -32,6 +32,7 @@
 // One row: greedy 7, top_k 20 17, top-p 29, launches of 1.5 us and the pick's chain.  Rows that
 // select_row does take 410 to 650.
 #include "fqa_common.h"
+#include "fqa_sample_bins.h"
 
 #include <cfloat>
 
@@ -380,12 +381,6 @@ __device__ __noinline__ int select_row(const float* lg, int N, uint32_t mk, doub
 }
 
 // ---- bins ----------------------------------------------------------------------------
-constexpr int kBins = 384;  // an eighth of an octave each: 48 octaves below the largest weight
-constexpr double kEightLog2e = 11.541560327111707;  // 8 log2(e)
-constexpr double kRound = 6755399441055744.0;       // 1.5 x 2^52: adding it rounds to an integer
-// Places that bins are used for: a row's of its largest logit, and a part's (one below these is none
-// that its row has bins for).  They and their differences fit int.
-constexpr double kMaxPlace = 536870912.0, kMaxPartPlace = 2 * kMaxPlace;
 constexpr int kNoBin = -(1 << 30);
 
 // 2^39 2^(r/8), |r| <= 1/2, to an integer: the polynomial through the Chebyshev points of degree 6,
@@ -419,12 +414,6 @@ struct BinWeight {
     return __builtin_bit_cast(u64, raised(r)) & 0xfffffffffffffull;
   }
 };
-// The bin of a logit at place l c, and its distance from the bin's middle; |l c| < 2^31.
-__device__ __forceinline__ int bin_of(double l, double c, double& r, double round = kRound) {
-  const double s = fma(l, c, round);
-  r = fma(l, c, round - s);
-  return (int)(uint32_t)__builtin_bit_cast(u64, s);
-}
 
 // ---- the parts -----------------------------------------------------------------------
 constexpr int kSThreads = 512;
@@ -434,10 +423,6 @@ constexpr int kPartLen = kSThreads * kPer;
 constexpr int kSmallK = 64;
 constexpr int kListCap = 256;             // a part's list; at most top_k where it would be longer
 constexpr int kBody = kBins + kBins / 2;  // masses, and counts of 32 bits
-// Copies of the histogram that a part's lanes add to: fewer of them wait for each other (2, 4 and 8
-// are within 1% of one another, at 16 their LDS leaves fewer workgroups to a CU).
-constexpr int kCols = 4;
-
 constexpr int kWordCap = 8192;  // logits of the cuts' bins that are selected from
 
 // What the parts make of a row together.
@@ -456,8 +441,8 @@ struct ScanLds {
   int widx[kSWaves];
   union {
     struct {
-      u64 mass[kBins * kCols];
-      uint32_t count[kBins * kCols];
+      u64 mass[kBins * kBinCols];
+      uint32_t count[kBins * kBinCols];
     } h;
     struct {
       u64 list[kListCap];
@@ -522,9 +507,9 @@ __global__ void __launch_bounds__(kSThreads, 8) filter_scan_kernel(FilterArgs a)
   const Settings st = settings_of(a, row);
   const bool lists = !st.greedy && st.k > 0 && st.k <= kSmallK, bins = !st.greedy && !lists;
   if (bins) {
-    for (int i = t; i < kBins * kCols; i += kSThreads) sh.h.mass[i] = 0;
+    for (int i = t; i < kBins * kBinCols; i += kSThreads) sh.h.mass[i] = 0;
     if (st.k > 0)
-      for (int i = t; i < kBins * kCols; i += kSThreads) sh.h.count[i] = 0;
+      for (int i = t; i < kBins * kBinCols; i += kSThreads) sh.h.count[i] = 0;
   } else if (t == 0) {
     sh.c.n = 0;
   }
@@ -648,8 +633,7 @@ __global__ void __launch_bounds__(kSThreads, 8) filter_scan_kernel(FilterArgs a)
     // the bins reach, the largest alone): what passes the comparison (NaN does not) is in the bins.
     const float mid = (float)((double)lo / c);
     const float low = fminf(logit_of(key_of(fmaxf(mid, -FLT_MAX)) + (mid > -FLT_MAX)), top);
-    u64* const mass = &sh.h.mass[-lo * kCols + (t & (kCols - 1))];
-    uint32_t* const count = &sh.h.count[-lo * kCols + (t & (kCols - 1))];
+    const uint32_t slots = slot_base(lo, t & (kBinCols - 1));
     const BinWeight bin_weight;
     double round = kRound;
     asm("" : "+s"(round));
@@ -657,14 +641,17 @@ __global__ void __launch_bounds__(kSThreads, 8) filter_scan_kernel(FilterArgs a)
 #pragma unroll
       for (int e = 0; e < kPer; ++e)
         if (x[e] >= low) {
-          const int b = bin_of((double)x[e], c, r, round) * kCols;
-          atomicAdd(mass + b, bin_weight(r));
-          atomicAdd(count + b, 1u);
+          const uint32_t at = bin_slot(bin_of((double)x[e], c, r, round), slots);
+          atomicAdd(&sh.h.mass[at], bin_weight(r));
+          atomicAdd(&sh.h.count[at], 1u);
         }
     } else {
 #pragma unroll
       for (int e = 0; e < kPer; ++e)
-        if (x[e] >= low) atomicAdd(mass + bin_of((double)x[e], c, r, round) * kCols, bin_weight(r));
+        if (x[e] >= low) {
+          const uint32_t at = bin_slot(bin_of((double)x[e], c, r, round), slots);
+          atomicAdd(&sh.h.mass[at], bin_weight(r));
+        }
     }
     head.w = hi;
   }
@@ -672,12 +659,12 @@ __global__ void __launch_bounds__(kSThreads, 8) filter_scan_kernel(FilterArgs a)
   if (t < kBins) {
     u64 mass = 0;
 #pragma unroll
-    for (int k = 0; k < kCols; ++k) mass += sh.h.mass[t * kCols + ((k + t) & (kCols - 1))];
+    for (int k = 0; k < kBinCols; ++k) mass += sh.h.mass[t * kBinCols + ((k + t) & (kBinCols - 1))];
     body[t] = mass;
     if (st.k > 0) {
       uint32_t n = 0;
 #pragma unroll
-      for (int k = 0; k < kCols; ++k) n += sh.h.count[t * kCols + ((k + t) & (kCols - 1))];
+      for (int k = 0; k < kBinCols; ++k) n += sh.h.count[t * kBinCols + ((k + t) & (kBinCols - 1))];
       reinterpret_cast<uint32_t*>(body + kBins)[t] = n;
     }
   }
