@@ -383,33 +383,21 @@ __device__ __noinline__ int select_row(const float* lg, int N, uint32_t mk, doub
 // ---- bins ----------------------------------------------------------------------------
 constexpr int kNoBin = -(1 << 30);
 
-// 2^39 2^(r/8), |r| <= 1/2, to an integer: the polynomial through the Chebyshev points of degree 6,
-// within 2^-41.6 of its value.  Its coefficients are kept in scalar registers (hidden from the
-// compiler, which would otherwise move each of them into vector registers for every weight).
+// bin_weight_raised with its coefficients in scalar registers (hidden from the compiler, which would
+// otherwise move each of them into vector registers for every weight).
 struct BinWeight {
   double c[6];
   __device__ __forceinline__ BinWeight() {
-    constexpr double s = 549755813888.0;  // 2^39
-    c[5] = s * 4.069351772310789e-08;
-    c[4] = s * 2.348396409244877e-06;
-    c[3] = s * 0.00010840646198027614;
-    c[2] = s * 0.0037535391505772045;
-    c[1] = s * 0.08664339756999671;
-    c[0] = s + 4503599627370496.0;  // + 2^52: the integer is in the low bits
 #pragma unroll
-    for (int i = 0; i < 6; ++i)
+    for (int i = 0; i < 6; ++i) {
+      c[i] = kBinWeight[i];
       if (i == 4)  // an instruction takes one scalar
         asm("" : "+v"(c[i]));
       else
         asm("" : "+s"(c[i]));
+    }
   }
-  __device__ __forceinline__ double raised(double r) const {  // by 2^52
-    double p = fma(r, c[5], c[4]);
-    p = fma(r, p, c[3]);
-    p = fma(r, p, c[2]);
-    p = fma(r, p, c[1]);
-    return fma(r, p, c[0]);
-  }
+  __device__ __forceinline__ double raised(double r) const { return bin_weight_raised(c, r); }
   __device__ __forceinline__ u64 operator()(double r) const {
     return __builtin_bit_cast(u64, raised(r)) & 0xfffffffffffffull;
   }

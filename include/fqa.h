@@ -591,8 +591,8 @@ int fqa_lora_add(const fqa_lora* w, const void* x, int64_t ldx, const int32_t* r
  *     at which the running sum of the kept weights reaches u[b] * (their mass), u[b] in [0, 1).
  * Logits of -inf and NaN are never picked, +inf ones share all of the weight; a row with nothing
  * to pick gives -1.  inv_temp NaN is greedy, top_p NaN >= 1, min_p NaN 0.  Weights are held to
- * 2^-41 of their value and summed exactly or in 64 bits; those below 2^-47 of the largest count as
- * nothing (but in a row with u = 0).  So the token is the one that exact arithmetic gives but for
+ * 2^-39 of their value and summed exactly or in 64 bits; those below 2^-47 of the largest may
+ * count as nothing (not in a row with u = 0).  So the token is the one that exact arithmetic gives but for
  * draws and cuts within ~(vocab 2^-47 + 1e-12) of a border, as shares of the kept mass, and it is
  * the same on every run.  vocab in [1, 2^24], n_rows in [0, 2^20], n_rows ceil(vocab / 10240) below
  * 2^23 - 16384.  `workspace`:

@@ -34,7 +34,21 @@ static int slots() {
   return 0;
 }
 
+// The largest error of a weight, relative to its value, over the distances from a bin's middle.
+static int weights() {
+  long double worst = 0;
+  const int n = 1 << 21;
+  for (int i = -n; i <= n; ++i) {
+    const double r = 0.5 * i / n;
+    const long double got = bin_weight_raised(kBinWeight, r) - kRaise;
+    worst = std::fmax(worst, std::fabs(got / (kBinUnit * std::exp2((long double)r / 8)) - 1));
+  }
+  std::printf("%.6Lg\n", worst);
+  return 0;
+}
+
 int main(int argc, char** argv) {
   if (argc == 2 && !std::strcmp(argv[1], "slots")) return slots();
+  if (argc == 2 && !std::strcmp(argv[1], "weights")) return weights();
   return 2;
 }

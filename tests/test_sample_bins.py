@@ -2,6 +2,8 @@
 the host by tests/cpp/sample_bins.cpp, built with UndefinedBehaviorSanitizer."""
 from __future__ import annotations
 
+import math
+import re
 import subprocess
 
 import pytest
@@ -31,3 +33,13 @@ def test_slots_of_far_places(bins):
     """Places up to 2^30: no term of a histogram index leaves its type."""
     n = int(bins("slots").split()[0])
     assert n > 100 * 384 * 4, n
+
+
+def test_weights_are_as_close_as_the_header_says(bins):
+    """The scan's weights against exp2 in 64 bits of significand: within what fqa.h states of them, and
+    not closer than a quarter of that (a stated bound is one that the code has)."""
+    text = (ROOT / "include" / "fqa.h").read_text()
+    stated = 2.0 ** -int(re.search(r"Weights are held to[\s*]+2\^-(\d+) of their value", text).group(1))
+    worst = float(bins("weights"))
+    print(f"worst relative error {worst:.3g} = 2^{math.log2(worst):.2f}, stated {stated:.3g}")
+    assert stated / 4 < worst <= stated
