@@ -193,8 +193,8 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
     else:
         nbytes = workspace.nbytes
-        if workspace.get_device() != index:
-            raise ValueError(f"workspace is on {workspace.device}, not on {x.device}")
+        if workspace.get_device() != index or not workspace.is_contiguous():
+            raise ValueError(f"workspace must be a contiguous tensor on {x.device}")
     launch(index, "fqa_lora_add", w_ref, x.data_ptr(), ldx, rows.data_ptr(), items.data_ptr(),
            meta.data_ptr(), rows_bound, item_bound_, y.data_ptr(), ldy, out.data_ptr(), ldo, f32,
            workspace.data_ptr(), nbytes)

@@ -54,8 +54,8 @@ def sample_filtered(logits: torch.Tensor, inv_temp: torch.Tensor, top_k: torch.T
         if need < 0:
             check(need, "fqa_sample_filtered_workspace_bytes")
         workspace = torch.empty(need or 16, dtype=torch.uint8, device=logits.device)
-    elif workspace.get_device() != index:
-        raise ValueError(f"workspace is on {workspace.device}, not on {logits.device}")
+    elif workspace.get_device() != index or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous tensor on {logits.device}")
     launch(index, "fqa_sample_filtered", logits.data_ptr(), B, N, logits.stride(0) if B > 1 else N,
            inv_temp.data_ptr(), top_k.data_ptr(), top_p.data_ptr(), min_p.data_ptr(), u.data_ptr(),
            out.data_ptr(), workspace.data_ptr(), workspace.nbytes)
