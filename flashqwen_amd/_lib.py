@@ -23,6 +23,7 @@ FQA_LORA_MAX_SLICES = 4
 FQA_LORA_MAX_RANK = 128
 FQA_LORA_MAX_ADAPTERS = 65536
 FQA_LORA_MAX_ITEMS = 16383
+FQA_LORA_MAX_COLS = 1 << 30
 FQA_LORA_META_LEN = 4
 FQA_PRE_TILE_Q = 64  # prefill rows per work item the step helpers plan with (fqa.h)
 

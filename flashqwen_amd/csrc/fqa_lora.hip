@@ -828,7 +828,8 @@ int check_weights(const fqa_lora* w) {
       w->n_in % 64)
     return FQA_EUNSUPPORTED;
   for (int s = 0, prev = 0; s < w->n_slices; prev = w->slice_end[s++])
-    if (w->slice_end[s] <= prev || (w->slice_end[s] - prev) % 64) return FQA_EUNSUPPORTED;
+    if (w->slice_end[s] <= prev || (w->slice_end[s] - prev) % 64 || w->slice_end[s] > FQA_LORA_MAX_COLS)
+      return FQA_EUNSUPPORTED;
   return FQA_OK;
 }
 

@@ -516,6 +516,7 @@ int fqa_qkv_proj_append(const fqa_dims* dims, const uint16_t* x, int64_t ldx,
 #define FQA_LORA_MAX_RANK 128
 #define FQA_LORA_MAX_ADAPTERS 65536
 #define FQA_LORA_MAX_ITEMS 16383
+#define FQA_LORA_MAX_COLS (1 << 30) /* n_out */
 #define FQA_LORA_META_LEN 4
 enum {
   FQA_LORA_META_ITEMS = 0,         /* items                                           */
@@ -537,7 +538,8 @@ typedef struct fqa_lora {
   int32_t n_in;         /* a multiple of 64                                              */
   int32_t n_slices;     /* 1..FQA_LORA_MAX_SLICES                                        */
   int32_t slice_end[FQA_LORA_MAX_SLICES]; /* output columns up to and with each slice,
-                                             every slice a multiple of 64 wide           */
+                                             every slice a multiple of 64 wide; n_out <=
+                                             FQA_LORA_MAX_COLS                           */
 } fqa_lora;
 
 /* The most items a plan of these bounds can have (item_cap, item_bound below). */
