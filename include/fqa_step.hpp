@@ -211,11 +211,11 @@ class StepContext {
   // The packed step's rows grouped by their requests' adapters (fqa_lora_plan), once per step:
   // adapter [requests of the batch] on the device, an id outside [0, n_adapters) for none.
   // `bounded`: for any batch within the context's bounds (a step captured with Pack), else for the
-  // batch last uploaded.
+  // batch last uploaded (one of more than max_rows rows, which the pack refuses, has none).
   void PlanAdapters(const int32_t* adapter, int n_adapters, hipStream_t stream,
                     bool bounded = false) {
     const int reqs = bounded ? slots_ : n_reqs_;
-    lora_bound_ = bounded ? max_rows_ : rows_;
+    lora_bound_ = bounded ? max_rows_ : std::min(rows_, max_rows_);
     lora_items_n_ = fqa_lora_item_bound(reqs, lora_bound_, n_adapters);
     Check(fqa_lora_plan(adapter, reqs, nullptr, cu_.D(), meta_.D(), reqs, lora_bound_, n_adapters,
                         lora_rows_.D(), lora_items_.D(), lora_items_n_, lora_meta_.D(), stream),
