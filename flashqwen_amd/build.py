@@ -111,12 +111,14 @@ def build_compat_driver() -> Path:
 
 
 def build_adapters_driver() -> Path:
-    """tests/cpp/adapters_cpp: adapters and filtered sampling through include/fqa_step.hpp."""
+    """tests/cpp/adapters_cpp, adapters_graph_cpp: adapters and filtered sampling through
+    include/fqa_step.hpp, eager and in a captured step."""
     root = PKG.parent
-    src = root / "tests" / "cpp" / "adapters_cpp.cpp"
-    exe = src.with_suffix("")
-    _run([HIPCC, "-O2", "-std=c++17", "-Wall", "-o", str(exe), str(src), f"-L{PKG}", "-lfqa",
-          "-Wl,-rpath,$ORIGIN/../../flashqwen_amd"])
+    for name in ("adapters_graph_cpp", "adapters_cpp"):
+        src = root / "tests" / "cpp" / (name + ".cpp")
+        exe = src.with_suffix("")
+        _run([HIPCC, "-O2", "-std=c++17", "-Wall", "-o", str(exe), str(src), f"-L{PKG}", "-lfqa",
+              "-Wl,-rpath,$ORIGIN/../../flashqwen_amd"])
     return exe
 
 
