@@ -148,7 +148,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     nb, Nb, R = b.shape
     ldx, cx = x.stride()
     ldy, cy = y.stride()
-    if rows_y != T or cx != 1 or cy != 1:
+    if rows_y != T or (T > 0 and (cx != 1 or cy != 1)):
         raise ValueError("x and y must have unit column stride and the same rows")
     slices = (N,) if slices is None else tuple(slices)
     S, total, ends = _ends(slices)
@@ -175,7 +175,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
         ldo = ldy
     else:
         ldo, co = out.stride()
-        if out.dtype is not y.dtype or co != 1 or out.size(0) != T or out.size(1) != N:
+        if out.dtype is not y.dtype or (co != 1 and T > 0) or out.size(0) != T or out.size(1) != N:
             raise ValueError("out must have y's dtype and shape and unit column stride")
         if T == 1:
             ldo = N

@@ -38,7 +38,7 @@ def sample_filtered(logits: torch.Tensor, inv_temp: torch.Tensor, top_k: torch.T
     """Tokens by temperature, top-k, top-p and min-p (fqa_sample_filtered): logits [B, N] fp32 (rows
     may be strided), inv_temp / top_p / min_p / u [B] fp32, top_k [B] int32 -> [B] int32 tokens, on
     the current stream of the logits' device; -1 for a row with nothing to pick."""
-    if logits.dtype != torch.float32 or logits.dim() != 2 or logits.stride(1) != 1:
+    if logits.dtype != torch.float32 or logits.dim() != 2 or (logits.stride(1) != 1 and logits.numel() > 0):
         raise ValueError("logits must be a 2-D fp32 tensor with unit column stride")
     index = logits.get_device()
     B, N = logits.shape

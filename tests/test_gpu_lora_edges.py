@@ -1,5 +1,5 @@
 """lora_add at the edges of what it takes: plans over adapters that the weights lack, infinities in the
-weights."""
+weights, no rows at all."""
 from __future__ import annotations
 
 import numpy as np
@@ -79,3 +79,22 @@ def test_infinities_in_the_weights(gpu, T_of, R, slices, f32):
     fine = np.isfinite(want)
     _check(torch.from_numpy(np.where(fine, g, 0.0)), np.where(fine, want, 0.0), np.where(fine, err, 0.0), f32,
            "finite columns")
+
+
+def test_no_rows_of_any_strides(gpu):
+    """Tensors without rows have no strides to speak of (numpy's come with zeros): nothing is launched."""
+    import torch
+
+    from flashqwen_amd.lora import lora_add, lora_plan
+    from flashqwen_amd.sample import sample_filtered
+
+    empty = lambda n, dt: torch.empty(0, n, dtype=dt, device=gpu).as_strided((0, n), (0, 0))  # noqa: E731
+    i32 = dict(dtype=torch.int32, device=gpu)
+    plan = lora_plan(torch.zeros(1, **i32), torch.zeros(2, **i32), _t(np.zeros(16, np.int32)), 2, 0)
+    a = torch.zeros(2, 16, 128, dtype=torch.bfloat16, device=gpu)
+    b = torch.zeros(2, 64, 16, dtype=torch.bfloat16, device=gpu)
+    x, y = empty(128, torch.bfloat16), empty(64, torch.bfloat16)
+    for out in (None, y, empty(64, torch.bfloat16)):
+        assert lora_add(y, x, a, b, torch.ones(2, device=gpu), plan, out=out).shape == (0, 64)
+    v = torch.zeros(0, device=gpu)
+    assert sample_filtered(empty(50, torch.float32), v, torch.zeros(0, **i32), v, v, v).shape == (0,)
