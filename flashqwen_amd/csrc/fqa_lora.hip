@@ -12,8 +12,8 @@
 //   o_proj 4096 -> 4096, 4 rows, rank 16         3.6 + 4.8
 //   q|k|v 4096 -> 6144, 64 rows, rank 16         5.3 + 5.2
 //   gate|up 4096 -> 24576, 250 rows, 64 adapters of rank 32     11 + 30   (3.0 TB/s of 124 MB)
-//   down 12288 -> 4096, 700 rows, rank 64        17.5 + 12.5  (x 17 MB and A 12.6 MB, from 100 CUs)
-//   q|k|v, 8192 rows, rank 64                    31 + 70   (y's 201 MB at 2.9 TB/s)
+//   down 12288 -> 4096, 700 rows, rank 64        17.6 + 12.6  (x 17 MB and A 12.6 MB, from 100 CUs)
+//   q|k|v, 8192 rows, rank 64                    31 + 72   (y's 201 MB at 2.8 TB/s, and h's planes)
 #include "fqa_common.h"
 
 namespace fqa {
@@ -659,11 +659,13 @@ struct Expand {
   }
 };
 
-// kColTile columns to a workgroup.  What bounds it: y's bytes, and at few rows the loads that wait for
-// one another (item, rank, B and h and y).  B's fragments are loaded first and stay in registers for
+// kColTile columns to a workgroup.  What bounds it: y's bytes and those of h, whose planes every
+// workgroup of columns reads and sums again (4 planes of 128 rows at rank 64: 131 KB, as much as its
+// tile of a bf16 y read and written), and at few rows the loads that wait for one another (item, rank, B
+// and h and y).  B's fragments are loaded first and stay in registers for
 // all of the item's rows (kJb: blocks of 16 ranks held), h goes through LDS once, and y_in of the next
-// 16 rows is on its way while those before are multiplied.  q|k|v at 8192 rows and rank 64: 70 us,
-// 201 MB of y at 2.9 TB/s.
+// 16 rows is on its way while those before are multiplied.  q|k|v at 8192 rows and rank 64: 72 us,
+// 201 MB of y at 2.8 TB/s.
 template <bool kF32, int kJb, int kRows>
 __global__ void __launch_bounds__(kLThreads, kJb > 4 ? 2 : kF32 && kJb > 2 ? 3 : 4)
 lora_expand_kernel(LoraArgs a) {
@@ -797,6 +799,9 @@ __global__ void __launch_bounds__(kLThreads, 3) lora_expand_few_kernel(LoraArgs 
 // the second product reads them all, and a chunk for every wave at least.  Both products of down at
 // 700 rows and rank 64 take 30 us with 8 splits, 37 with 12 and 34 with 16; of q|k|v at 8192 rows and
 // rank 64 99 by tiles in 4 splits, 114 in 2, 117 in 8 and 117 without tiles.
+// All of it goes by the call's bounds, since the host does not know the items: a decode step planned by
+// bounds of 8192 rows and 256 requests takes the forms for many rows (o_proj at 4 rows 9.7 us where its
+// own bounds take 7.8, gate|up at 250 rows 47.7 and 34.5, q|k|v at 64 rows of rank 64 31.4 and 18.5).
 constexpr int kShrinkWgs = 512, kTileWgs = 300, kMaxSplits = 8;
 struct Cut {
   bool few, tile;
